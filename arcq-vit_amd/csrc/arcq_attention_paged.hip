@@ -25,9 +25,11 @@
 // registers 8 i .. 8 i + 7 are one 16-byte piece of a page (eight bytes of one).  So are the eight values of a key row: a page's layout
 // is that of the operands, both are loaded from memory into operand registers, 512 bytes of consecutive addresses for 32 lanes.
 //
-// FP8 pages: a key's exponent belongs to its row of K, one lane, and is applied as the values are widened (exact); a value's belongs
-// to a column of P^T, and is applied to the probabilities.  fp16 probabilities carry a factor of 2^8 that cancels in the end: the largest
-// exponent (7) then reaches 2^15, and many small ones behind one large, or small exponents, stay above its subnormals for longer.
+// FP8 pages: a key's exponent belongs to its row of K, one lane, and is applied as the values are widened (exact).  A value's belongs to a column
+// of P^T.  With bf16 it is applied to the probabilities; fp16 has no room for that (2^-14 of a probability leaves its normal numbers at 2^-8 of
+// the largest: 65 536 keys of values of 0.01 behind one of a score 12 higher were off by 24 %), so there every value is widened with
+// its own exponent (exact), which is then no longer a part of the probabilities' range.  fp16 probabilities carry a factor of 2^8 that cancels in
+// the end: many small ones behind one large stay above its subnormals for longer.
 #include "arcq_gemm.h"
 #include "arcq_kv_pages.h"
 
@@ -40,8 +42,7 @@ constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kNegInf = -__builtin_inff();
 // How far a score may be above the reference (in powers of two) before that follows.
 template <typename T, bool F8> constexpr float kSlack = 16.0f;
-template <> constexpr float kSlack<_Float16, false> = 6.0f;
-template <> constexpr float kSlack<_Float16, true> = 0.0f;
+template <bool F8> constexpr float kSlack<_Float16, F8> = 6.0f;
 template <typename T> constexpr float kShift = 0.0f;
 template <> constexpr float kShift<_Float16> = 8.0f;
 
@@ -240,7 +241,34 @@ __device__ __forceinline__ u32x4_t widen(uint32_t lo, uint32_t hi, float scale, 
     o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
     return o;
 }
+// FP8 pages: the values' exponents are applied as they are widened, else to the probabilities.
+template <typename T, bool F8> constexpr bool kScaleValues = false;
+template <> constexpr bool kScaleValues<_Float16, true> = true;
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, static_cast<uint32_t>(127 + e) << 23); }
+
+typedef short short2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ int exponent_of(const u32x4_t &e, int i) { return __builtin_amdgcn_sbfe(static_cast<int>(e[i >> 2]), 8 * (i & 3), 8); }
+// fp16: the powers of two of two tokens' values, times 2^8, so that those of fp16 rows (exponents -14 to 7) are normal numbers.  Pages that were
+// written from another type: zero below -22, infinity above 7.  An exponent's byte goes to the top of 16 bits, then to fp16's field.
+__device__ __forceinline__ half2_t scales_of(uint32_t e, bool upper)               // (of the upper two of four exponents)
+{
+    const uint32_t two = __builtin_amdgcn_perm(0u, e, upper ? 0x030c020cu : 0x010c000cu);
+    const short2_t top = __builtin_elementwise_min(__builtin_elementwise_max(__builtin_bit_cast(short2_t, two), short2_t{-23 * 256, -23 * 256}),
+                                                   short2_t{8 * 256, 8 * 256});
+    return __builtin_bit_cast(half2_t, __builtin_bit_cast(ushort2_t, top) * ushort2_t{4, 4} + ushort2_t{23 << 10, 23 << 10});
+}
+// Eight FP8 values, each times its token's power of two: exact (2^-8 of an FP8 value is fp16's).
+__device__ __forceinline__ u32x4_t widen_each(uint32_t lo, uint32_t hi, const half2_t *scale)
+{
+    u32x4_t o = widen(lo, hi, 1.0f / 256.0f, _Float16{});
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t two = o[i];                 // (a copy: a bit cast of a vector's element takes the first one)
+        o[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, two) * scale[i]);
+    }
+    return o;
+}
 
 // The token behind row m of a 32-key block of K.
 template <bool F8>
@@ -558,6 +586,7 @@ paged_rows_kernel(const PagedArgs a)
             if constexpr (F8) {
 #pragma unroll
                 for (int i = 0; i < NB; ++i) keep_tokens<F8>(vreg[i], base + 16 * lh, t.lo, t.hi);
+                keep_tokens<F8>(vexp, base + 16 * lh, t.lo, t.hi);
             } else {
 #pragma unroll
                 for (int i = 0; i < 2 * NB; ++i) keep_tokens<F8>(vreg[i], base + 16 * (i / NB) + 8 * lh, t.lo, t.hi);
@@ -588,15 +617,20 @@ paged_rows_kernel(const PagedArgs a)
         for (int v = 0; v < 16; ++v) {
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.c2, shift));
             l += p;
-            s[v] = F8 ? __builtin_amdgcn_ldexpf(p, __builtin_amdgcn_sbfe(static_cast<int>(vexp[v >> 2]), 8 * (v & 3), 8)) : p;
+            s[v] = F8 && !kScaleValues<T, F8> ? __builtin_amdgcn_ldexpf(p, exponent_of(vexp, v)) : p;
         }
+        half2_t vscale[8];
+        if constexpr (kScaleValues<T, F8>)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) vscale[i] = scales_of(vexp[i >> 1], i & 1);
         u32x4_t pf[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) pf[i][e] = pack2(s[8 * i + 2 * e], s[8 * i + 2 * e + 1], T{});
         auto value = [&](int i, int j) {
-            if constexpr (F8) return widen(vreg[j][2 * i], vreg[j][2 * i + 1], 1.0f, T{});
+            if constexpr (kScaleValues<T, F8>) return widen_each(vreg[j][2 * i], vreg[j][2 * i + 1], vscale + 4 * i);
+            else if constexpr (F8) return widen(vreg[j][2 * i], vreg[j][2 * i + 1], 1.0f, T{});
             else return vreg[i * NB + j];
         };
 #pragma unroll
@@ -744,8 +778,10 @@ paged_tile_kernel(const PagedArgs a)
     constexpr int LOADS = HALF / 1024;             // 1 KB loads of each half
     constexpr int MINE = (LOADS + 3) / 4;          // a wave's (some are loaded twice where they do not divide)
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];      // [2][keys, values, exponents]
+    __shared__ half2_t scales[kScaleValues<T, F8> ? 4 : 1][32];                 // each wave's, of a block's values
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lr = lane & 31, lh = lane >> 5;
+    half2_t *wave_scales = scales[kScaleValues<T, F8> ? wave : 0];
     const int place = a.by_kv_heads(blockIdx.x), kv = blockIdx.x - place * a.kv_heads;
     Item t;
     if (!find_item<kTileRows, 6>(a, place, lane, t)) return;
@@ -892,7 +928,7 @@ paged_tile_kernel(const PagedArgs a)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 kscale[h] = power_of_two(static_cast<int8_t>(block[2 * HALF + 32 * h + ktok]));
-                vexp[h] = *reinterpret_cast<const u32x4_t *>(block + 2 * HALF + 64 + 32 * h + 16 * lh);
+                if constexpr (!kScaleValues<T, F8>) vexp[h] = *reinterpret_cast<const u32x4_t *>(block + 2 * HALF + 64 + 32 * h + 16 * lh);
             }
         }
         const int base = kb * 64;
@@ -915,6 +951,16 @@ paged_tile_kernel(const PagedArgs a)
         }
         if (careful) break;                       // (the same in all waves)
         if (base >= wave_hi || base + 64 <= wave_lo) continue;
+        if constexpr (kScaleValues<T, F8>) {
+            // A lane a pair of tokens, for all lanes of the wave: each for its own 32 tokens took 42 us in place of 39 (64 dims, a window of 1 000).
+            // (What lies outside of the tile's keys, where an exponent may be anything: zero times zero.)
+            const int first = base + 2 * lr;
+            half2_t two = scales_of(*reinterpret_cast<const uint16_t *>(block + 2 * HALF + 64 + 2 * lr), false);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) two[i] = first + i >= t.lo && first + i < t.hi ? two[i] : static_cast<_Float16>(0.0f);
+            if (lh == 0) wave_scales[lr] = two;
+            __builtin_amdgcn_wave_barrier();          // (the wave's own, and its LDS accesses keep their order)
+        }
         const unsigned char *kt = block + (lh * 64 + ktok) * 16;
         const unsigned char *vt = block + HALF + lr * 16;
         float16_t s[2];
@@ -964,8 +1010,12 @@ paged_tile_kernel(const PagedArgs a)
             for (int v = 0; v < 16; ++v) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][v], a.c2, shift));
                 l += p;
-                s[h][v] = F8 ? __builtin_amdgcn_ldexpf(p, __builtin_amdgcn_sbfe(static_cast<int>(vexp[h][v >> 2]), 8 * (v & 3), 8)) : p;
+                s[h][v] = F8 && !kScaleValues<T, F8> ? __builtin_amdgcn_ldexpf(p, exponent_of(vexp[h], v)) : p;
             }
+            half2_t vscale[8];
+            if constexpr (kScaleValues<T, F8>)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) vscale[i] = wave_scales[16 * h + 8 * lh + i];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -974,8 +1024,13 @@ paged_tile_kernel(const PagedArgs a)
             for (int j = 0; j < NB; ++j) {
                 if constexpr (F8) {
                     const u32x4_t w = *reinterpret_cast<const u32x4_t *>(vt + ((2 * h + lh) * D + 32 * j) * 16);
-                    o[j] = mfma(widen(w[0], w[1], 1.0f, T{}), pf[0], o[j], T{});
-                    o[j] = mfma(widen(w[2], w[3], 1.0f, T{}), pf[1], o[j], T{});
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        u32x4_t v;
+                        if constexpr (kScaleValues<T, F8>) v = widen_each(w[2 * i], w[2 * i + 1], vscale + 4 * i);
+                        else v = widen(w[2 * i], w[2 * i + 1], 1.0f, T{});
+                        o[j] = mfma(v, pf[i], o[j], T{});
+                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
