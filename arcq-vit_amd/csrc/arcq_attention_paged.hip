@@ -28,23 +28,25 @@
 // FP8 pages: a key's exponent belongs to its row of K, one lane, and is applied as the values are widened (exact).  A value's belongs to a column
 // of P^T.  With bf16 it is applied to the probabilities; fp16 has no room for that (2^-14 of a probability leaves its normal numbers at 2^-8 of
 // the largest: 65 536 keys of values of 0.01 behind one of a score 12 higher were off by 24 %), so there every value is widened with
-// its own exponent (exact), which is then no longer a part of the probabilities' range.  fp16 probabilities carry a factor of 2^8 that cancels in
-// the end: many small ones behind one large stay above its subnormals for longer.
+// its own exponent (exact), which is then no longer a part of the probabilities' range.
+//
+// Range.  Probabilities carry a factor 2^shift, FP8 values of bf16 another (Range below); both cancel in the end.  fp16: 2^8, so that many small
+// probabilities behind one large stay above its subnormals for longer.  bf16: as small as keeps the sum of n keys finite in fp32 whatever
+// finite values they have: the mean of values near the type's end is finite, its numerator need not be.  (What that takes from the other end: a term
+// keeps all of fp32's bits while probability times value is above 2^-125 n 2^kSlack, 2^-106 for 8 192 keys.)
 #include "arcq_gemm.h"
 #include "arcq_kv_pages.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace arcq {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kNegInf = -__builtin_inff();
-// How far a score may be above the reference (in powers of two) before that follows.
-template <typename T, bool F8> constexpr float kSlack = 16.0f;
-template <bool F8> constexpr float kSlack<_Float16, F8> = 6.0f;
-template <typename T> constexpr float kShift = 0.0f;
-template <> constexpr float kShift<_Float16> = 8.0f;
+// How far a score may be above the reference (in powers of two) before that follows, in the kernel of many rows.
+constexpr int kSlack = 6;
 
 // Division of 0 .. 2^30 - 1 by a number known on the host: l = ceil(log2 d), m = ceil(2^(30 + l) / d) < 2^32; m d exceeds 2^(30 + l) by less
 // than 2^l, n times that by less than 2^(30 + l), so the quotient is exact.
@@ -62,6 +64,22 @@ struct Divide {
     __device__ __forceinline__ int operator()(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * m) >> shift); }
 };
 
+// The factors of probabilities (2^shift) and of FP8 values whose exponents go to the probabilities (value_scale); back: the latter's inverse, for
+// the result.  bf16, sums of up to 2^n keys, probabilities of up to 2^(shift + slack):
+//   16-bit pages  2^n * 2^(shift + slack) * |v| < 2^128 / 2
+//   FP8           P = p 2^e is a bf16 number at both ends of e, 2^(119 + 8) and 2^(-110 + 8 - slack) less 18 powers;  2^n * 2^127 * 448 * value_scale < 2^128
+struct Range {
+    float shift, value_scale, back;
+    Range(int dtype, bool f8, int64_t keys, int slack)
+    {
+        const int n = log2_of(std::max<int64_t>(keys, 1));
+        const bool scaled = dtype == ARCQ_BF16 && f8;
+        shift = static_cast<float>(dtype == ARCQ_F16 ? 8 : f8 ? 8 - slack : -(n + slack + 1));
+        value_scale = scaled ? std::ldexp(1.0f, -(n + 9)) : 1.0f;
+        back = scaled ? std::ldexp(1.0f, n + 9) : 1.0f;
+    }
+};
+
 struct PagedArgs {
     const unsigned char *kp, *vp;
     const int8_t *ke, *ve;
@@ -76,6 +94,7 @@ struct PagedArgs {
     int q_heads, kv_heads, group, sequences, page_shift, window, causal;
     int slots, min_blocks;           // items that the chip takes at once for each key head (0: tiles are not split), and the least blocks of one
     float c2;                        // scale * log2(e)
+    float shift, value_scale, back;  // Range
     Divide by_group, by_kv_heads, by_q_heads;
 };
 
@@ -344,7 +363,7 @@ __device__ __forceinline__ void store_rows(const PagedArgs &a, const Item &t, in
     const int tok = a.by_group(row), head = kv * a.group + row - tok * a.group;
     const int64_t token = static_cast<int64_t>(t.token0) + tok;
     if (t.parts == 1) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? 0.0f : a.back / l;
         unsigned char *dst = a.out + token * a.out_token + head * a.out_head;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
@@ -409,7 +428,7 @@ __device__ __forceinline__ void careful_tile(const PagedArgs &a, const Item &t, 
             for (int x = 32; x; x >>= 1) bm = fmaxf(bm, __shfl_xor(bm, x));
             const float m_new = fmaxf(m, bm), base2 = m_new == kNegInf ? 0.0f : m_new;
             const float alpha = __builtin_amdgcn_exp2f(m - base2);
-            const float p = lane < n ? __builtin_amdgcn_exp2f(s - base2 + kShift<T>) : 0.0f;
+            const float p = lane < n ? __builtin_amdgcn_exp2f(s - base2 + a.shift) : 0.0f;
             float sum = p;
 #pragma unroll
             for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
@@ -424,11 +443,11 @@ __device__ __forceinline__ void careful_tile(const PagedArgs &a, const Item &t, 
                 const unsigned char *v = a.vp + (sj - oj) * (D * SZ) + oj / W * D * 16 + oj % W * SZ;
 #pragma unroll
                 for (int i = 0; i < PER; ++i)
-                    if (lane + 64 * i < D) o[i] = __builtin_fmaf(pj, value(v + (lane + 64 * i) * 16, ej), o[i]);
+                    if (lane + 64 * i < D) o[i] = __builtin_fmaf(pj, value(v + (lane + 64 * i) * 16, ej) * a.value_scale, o[i]);
             }
         }
         const bool alone = t.parts == 1;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? 0.0f : a.back / l;
         T *dst = reinterpret_cast<T *>(a.out + token * a.out_token + head * a.out_head);
         const int64_t at = part_row<TILE>(a, t, kv, t.part, r) * D;
 #pragma unroll
@@ -612,7 +631,7 @@ paged_rows_kernel(const PagedArgs a)
                 for (int v = 0; v < 16; ++v) o[i][v] *= alpha;
             m = m_new;
         }
-        const float shift = kShift<T> - base2;
+        const float shift = a.shift - base2;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.c2, shift));
@@ -630,7 +649,7 @@ paged_rows_kernel(const PagedArgs a)
             for (int e = 0; e < 4; ++e) pf[i][e] = pack2(s[8 * i + 2 * e], s[8 * i + 2 * e + 1], T{});
         auto value = [&](int i, int j) {
             if constexpr (kScaleValues<T, F8>) return widen_each(vreg[j][2 * i], vreg[j][2 * i + 1], vscale + 4 * i);
-            else if constexpr (F8) return widen(vreg[j][2 * i], vreg[j][2 * i + 1], 1.0f, T{});
+            else if constexpr (F8) return widen(vreg[j][2 * i], vreg[j][2 * i + 1], a.value_scale, T{});
             else return vreg[i * NB + j];
         };
 #pragma unroll
@@ -680,7 +699,7 @@ paged_rows_kernel(const PagedArgs a)
         const int rtok = a.by_group(rr), rhead = kv * a.group + rr - rtok * a.group;
         const int64_t token = static_cast<int64_t>(t.token0) + rtok;
         const bool alone = t.parts == 1;
-        const float inv = alone ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f;
+        const float inv = alone ? (total == 0.0f ? 0.0f : a.back / total) : 1.0f;
         const int64_t at = part_row<32>(a, t, kv, t.part, r);
         float *po = alone ? nullptr : a.part_o + at * D;
         unsigned char *dst = a.out + token * a.out_token + rhead * a.out_head;
@@ -990,9 +1009,9 @@ paged_tile_kernel(const PagedArgs a)
         float bm = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
         for (int v = 1; v < 16; ++v) bm = fmaxf(fmaxf(s[0][v], s[1][v]), bm);
-        // The reference is left where it is while no score is more than 2^kSlack above it: probabilities are relative, and every type of theirs
-        // has room for that.
-        if (__any(bm * a.c2 > m + kSlack<T, F8>)) {
+        // The reference is left where it is while no score is more than kSlack above it: probabilities are relative, and `shift` leaves room for
+        // 2^kSlack in theirs, their sums' and their products' types.
+        if (__any(bm * a.c2 > m + static_cast<float>(kSlack))) {
             const float m_new = fmaxf(m, max_halves(bm) * a.c2);
             const float alpha = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
             l *= alpha;
@@ -1002,7 +1021,7 @@ paged_tile_kernel(const PagedArgs a)
                 for (int v = 0; v < 16; ++v) o[i][v] *= alpha;
             m = m_new;
         }
-        const float shift = kShift<T> - (m == kNegInf ? 0.0f : m);     // (a row that has seen nothing yet)
+        const float shift = a.shift - (m == kNegInf ? 0.0f : m);       // (a row that has seen nothing yet)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             u32x4_t pf[2];
@@ -1028,7 +1047,7 @@ paged_tile_kernel(const PagedArgs a)
                     for (int i = 0; i < 2; ++i) {
                         u32x4_t v;
                         if constexpr (kScaleValues<T, F8>) v = widen_each(w[2 * i], w[2 * i + 1], vscale + 4 * i);
-                        else v = widen(w[2 * i], w[2 * i + 1], 1.0f, T{});
+                        else v = widen(w[2 * i], w[2 * i + 1], a.value_scale, T{});
                         o[j] = mfma(v, pf[i], o[j], T{});
                     }
                 } else {
@@ -1093,7 +1112,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] += o[i];
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const float inv = total == 0.0f ? 0.0f : a.back / total;
     const int head = static_cast<int>(at - token * a.q_heads);
     u32x2_t w;
     w[0] = pack2(sum[0] * inv, sum[1] * inv, T{});
@@ -1266,6 +1285,9 @@ ARCQ_API int arcq_attention_paged_fwd(const arcq_attention_paged_args *p, void *
     a.sequences = static_cast<int>(p->sequences), a.page_shift = log2_of(p->pages.page_size);
     a.window = static_cast<int>(std::min<int64_t>(p->window, 1 << 30)), a.causal = p->causal ? 1 : 0, a.slots = plan.slots, a.min_blocks = plan.min_blocks;
     a.c2 = p->scale * kLog2e;
+    const int64_t most = p->table_width * p->pages.page_size;
+    const Range range(p->dtype, p->pages.dtype == ARCQ_FP8, p->window ? std::min(most, p->window) : most, plan.tile ? kSlack : 0);
+    a.shift = range.shift, a.value_scale = range.value_scale, a.back = range.back;
     a.by_group = Divide(a.group), a.by_kv_heads = Divide(a.kv_heads), a.by_q_heads = Divide(a.q_heads);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int64_t dim = p->pages.head_dim;
