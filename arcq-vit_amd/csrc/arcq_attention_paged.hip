@@ -45,6 +45,9 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kNegInf = -__builtin_inff();
+// A row's maximum: kNegInf if it sees no key (its result is zero), kLowest if it sees some and none has a score above minus infinity (0 / 0).
+constexpr float kLowest = -3.402823466e38f;
+__device__ __forceinline__ float row_maximum(float m, bool sees) { return sees ? fmaxf(m, kLowest) : m; }
 // How far a score may be above the reference (in powers of two) before that follows, in the kernel of many rows.
 constexpr int kSlack = 6;
 
@@ -363,7 +366,7 @@ __device__ __forceinline__ void store_rows(const PagedArgs &a, const Item &t, in
     const int tok = a.by_group(row), head = kv * a.group + row - tok * a.group;
     const int64_t token = static_cast<int64_t>(t.token0) + tok;
     if (t.parts == 1) {
-        const float inv = l == 0.0f ? 0.0f : a.back / l;
+        const float inv = m == kNegInf ? 0.0f : a.back / l;
         unsigned char *dst = a.out + token * a.out_token + head * a.out_head;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
@@ -407,6 +410,7 @@ __device__ __forceinline__ void careful_tile(const PagedArgs &a, const Item &t, 
             hi = min(max(t.len - t.queries + tok + 1, 0), t.len);
             if (a.window) lo = max(t.len - t.queries + tok + 1 - a.window, 0);
         }
+        const bool sees = hi > lo;
         lo = max(lo, t.k0 << SHIFT), hi = min(hi, t.k1 << SHIFT);
         const T *q = reinterpret_cast<const T *>(a.q + token * a.q_token + head * a.q_head);
         float m = kNegInf, l = 0.0f, o[PER];
@@ -446,8 +450,9 @@ __device__ __forceinline__ void careful_tile(const PagedArgs &a, const Item &t, 
                     if (lane + 64 * i < D) o[i] = __builtin_fmaf(pj, value(v + (lane + 64 * i) * 16, ej) * a.value_scale, o[i]);
             }
         }
+        m = row_maximum(m, sees);
         const bool alone = t.parts == 1;
-        const float inv = l == 0.0f ? 0.0f : a.back / l;
+        const float inv = m == kNegInf ? 0.0f : a.back / l;
         T *dst = reinterpret_cast<T *>(a.out + token * a.out_token + head * a.out_head);
         const int64_t at = part_row<TILE>(a, t, kv, t.part, r) * D;
 #pragma unroll
@@ -664,6 +669,7 @@ paged_rows_kernel(const PagedArgs a)
         return;
     }
 
+    m = row_maximum(m, hi > lo);
     if constexpr (WAVES == 1) {
         if (live) store_rows<T, D>(a, t, kv, row, lh, m, l, o);
         return;
@@ -699,7 +705,7 @@ paged_rows_kernel(const PagedArgs a)
         const int rtok = a.by_group(rr), rhead = kv * a.group + rr - rtok * a.group;
         const int64_t token = static_cast<int64_t>(t.token0) + rtok;
         const bool alone = t.parts == 1;
-        const float inv = alone ? (total == 0.0f ? 0.0f : a.back / total) : 1.0f;
+        const float inv = alone ? (mm == kNegInf ? 0.0f : a.back / total) : 1.0f;
         const int64_t at = part_row<32>(a, t, kv, t.part, r);
         float *po = alone ? nullptr : a.part_o + at * D;
         unsigned char *dst = a.out + token * a.out_token + rhead * a.out_head;
@@ -1064,7 +1070,7 @@ paged_tile_kernel(const PagedArgs a)
         return;
     }
     l += __shfl_xor(l, 32);
-    if (live) store_rows<T, D, kTileRows>(a, t, kv, row, lh, m, l, o);
+    if (live) store_rows<T, D, kTileRows>(a, t, kv, row, lh, row_maximum(m, hi > lo), l, o);
 }
 
 // ---- the parts of a row, joined: a workgroup has a row, groups of D / 4 threads take the parts in turn and are added in their order (the
@@ -1112,7 +1118,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] += o[i];
     }
-    const float inv = total == 0.0f ? 0.0f : a.back / total;
+    const float inv = mm == kNegInf ? 0.0f : a.back / total;
     const int head = static_cast<int>(at - token * a.q_heads);
     u32x2_t w;
     w[0] = pack2(sum[0] * inv, sum[1] * inv, T{});
