@@ -17,6 +17,7 @@ import math
 from typing import List, NamedTuple, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import ARCQ_F16, ARCQ_F32
@@ -842,8 +843,12 @@ def kv_cache_pages(num_pages: int, heads: int, head_dim: int, page_size: int = 6
 
 
 def _no_grad(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    _check(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)),
+    given = [t for t in tensors if t is not None]
+    _check(not (torch.is_grad_enabled() and any(t.requires_grad for t in given)),
            f"{name} has no backward pass: call it under torch.no_grad() or on tensors without gradient")
+    # (no_grad does not switch forward mode off)
+    _check(all(forward_ad.unpack_dual(t).tangent is None for t in given),
+           f"{name} has no backward pass and no forward-mode derivative: call it on tensors without tangents")
 
 
 def _same_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
