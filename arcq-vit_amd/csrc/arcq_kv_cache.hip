@@ -359,7 +359,8 @@ int cache_checked(const char *fn, const arcq_kv_cache_args *p, bool write, void 
     if (const int rc = check_page_pointers(fn, p->pages)) return rc;
     if (!aligned(p->k, 16) || !aligned(p->v, 16) || p->k_row_stride % 8 || p->k_head_stride % 8 || p->v_row_stride % 8 || p->v_head_stride % 8)
         return fail(ARCQ_ERR_ALIGN, "%s: every row of k and v must be 16-byte aligned", fn);
-    if (p->rows >= (int64_t(1) << 29)) return fail(ARCQ_ERR_SHAPE, "%s: too many rows", fn);
+    // (a grid's axis holds fewer than 2^32 threads: at 32 rows a workgroup of 256 fewer than 2^24 workgroups)
+    if (p->rows > ((int64_t(1) << 24) - 1) * 32) return fail(ARCQ_ERR_SHAPE, "%s: too many rows", fn);
     CacheArgs a{};
     a.kp = static_cast<unsigned char *>(p->pages.k), a.vp = static_cast<unsigned char *>(p->pages.v);
     a.ke = p->pages.k_exponents, a.ve = p->pages.v_exponents;
@@ -368,7 +369,7 @@ int cache_checked(const char *fn, const arcq_kv_cache_args *p, bool write, void 
     a.k_row = 2 * p->k_row_stride, a.k_head = 2 * p->k_head_stride, a.v_row = 2 * p->v_row_stride, a.v_head = 2 * p->v_head_stride;
     a.heads = static_cast<int>(p->pages.heads), a.dim = static_cast<int>(p->pages.head_dim), a.page_shift = log2_of(p->pages.page_size);
     const bool f8 = p->pages.dtype == ARCQ_FP8;
-    // (a grid's axis holds fewer than 2^32 threads: 2^29 rows) Rows of a workgroup, and up to W - 1 more (at most kRows); few rows: fewer, so that more of the chip takes part.
+    // Rows of a workgroup, and up to W - 1 more (at most kRows); few rows: fewer, so that more of the chip takes part.
     a.run = a.rows * a.heads >= int64_t(32) * 4 * device_cus() ? 32 : 16;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (p->dtype == ARCQ_F16) f8 ? launch_cache<_Float16, true>(a, write, st) : launch_cache<_Float16, false>(a, write, st);

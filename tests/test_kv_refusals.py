@@ -119,6 +119,14 @@ def test_grids_of_more_threads_than_an_axis_holds_are_refused():
     assert lib.arcq_qk_norm_rotary(ctypes.byref(_rotary(tokens=1 << 62, q_heads=2, k_heads=2)), None) == -4
 
 
+@pytest.mark.parametrize("rows", [(1 << 29) - 31, (1 << 29) - 1])
+def test_rows_whose_workgroups_just_fill_an_axis_are_refused(rows):
+    """32 rows a workgroup of 256 threads: from 2^29 - 31 rows on there are 2^24 workgroups, 2^32 threads, one more than an axis holds."""
+    lib = _lib.load()
+    for fn in (lib.arcq_kv_cache_write, lib.arcq_kv_cache_read):
+        assert fn(ctypes.byref(_cache(rows=rows)), None) == -4 and b"too many rows" in lib.arcq_last_error()
+
+
 def test_a_window_of_any_size_is_the_longest_one():
     lib = _lib.load()
     sizes = [lib.arcq_attention_paged_workspace(ctypes.byref(_attention(table_width=4096, window=w))) for w in (0, 1 << 30, (1 << 63) - 1)]
