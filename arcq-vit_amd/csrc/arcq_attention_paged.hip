@@ -1269,7 +1269,8 @@ ARCQ_API int arcq_attention_paged_fwd(const arcq_attention_paged_args *p, void *
     if (!p->q || !p->out || !p->q_offsets || !p->kv_lengths || (p->table_width && !p->page_table)) return fail(ARCQ_ERR_NULL, "%s: NULL tensor pointer", fn);
     if (const int rc = check_page_pointers(fn, p->pages)) return rc;
     if (p->pages.num_pages == 0 && p->table_width) return fail(ARCQ_ERR_SHAPE, "%s: a page table without pages", fn);
-    if (!aligned(p->q, 16) || !aligned(p->out, 16) || p->q_token_stride % 8 || p->q_head_stride % 8 || p->out_token_stride % 8 || p->out_head_stride % 8)
+    if (!rows_aligned(p->q, p->tokens, p->q_token_stride, p->q_heads, p->q_head_stride) ||
+        !rows_aligned(p->out, p->tokens, p->out_token_stride, p->q_heads, p->out_head_stride))
         return fail(ARCQ_ERR_ALIGN, "%s: every row of q and out must be 16-byte aligned", fn);
     const Plan plan = plan_of(p);
     if (plan.slots && (!p->workspace || !aligned(p->workspace, 16))) return fail(ARCQ_ERR_NULL, "%s: workspace missing or not 16-byte aligned", fn);

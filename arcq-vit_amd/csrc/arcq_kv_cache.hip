@@ -357,7 +357,8 @@ int cache_checked(const char *fn, const arcq_kv_cache_args *p, bool write, void 
     if (p->rows == 0 || p->pages.heads == 0) return ARCQ_OK;
     if (!p->k || !p->v || !p->slots) return fail(ARCQ_ERR_NULL, "%s: NULL tensor pointer", fn);
     if (const int rc = check_page_pointers(fn, p->pages)) return rc;
-    if (!aligned(p->k, 16) || !aligned(p->v, 16) || p->k_row_stride % 8 || p->k_head_stride % 8 || p->v_row_stride % 8 || p->v_head_stride % 8)
+    if (!rows_aligned(p->k, p->rows, p->k_row_stride, p->pages.heads, p->k_head_stride) ||
+        !rows_aligned(p->v, p->rows, p->v_row_stride, p->pages.heads, p->v_head_stride))
         return fail(ARCQ_ERR_ALIGN, "%s: every row of k and v must be 16-byte aligned", fn);
     // (a grid's axis holds fewer than 2^32 threads: at 32 rows a workgroup of 256 fewer than 2^24 workgroups)
     if (p->rows > ((int64_t(1) << 24) - 1) * 32) return fail(ARCQ_ERR_SHAPE, "%s: too many rows", fn);

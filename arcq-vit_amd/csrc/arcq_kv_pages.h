@@ -68,6 +68,11 @@ inline int check_page_pointers(const char *fn, const arcq_kv_pages &p)
         return fail(ARCQ_ERR_ALIGN, "%s: pages must be 16-byte aligned", fn);
     return ARCQ_OK;
 }
+// Do all rows [rows, heads] of 16-bit values lie on 16-byte boundaries?  (A dimension of one entry has any stride.)
+inline bool rows_aligned(const void *p, int64_t rows, int64_t row_stride, int64_t heads, int64_t head_stride)
+{
+    return aligned(p, 16) && (rows <= 1 || row_stride % 8 == 0) && (heads <= 1 || head_stride % 8 == 0);
+}
 inline int log2_of(int64_t power)
 {
     int n = 0;

@@ -400,7 +400,10 @@ ARCQ_API int arcq_qk_norm_rotary(const arcq_qk_norm_rotary_args *p, void *stream
                                 p->k_token_stride, p->k_head_stride, p->k_out_token_stride, p->k_out_head_stride};
     const int size = p->dtype == ARCQ_F32 ? 4 : 2;
     bool rows = p->head_dim % 16 == 0;
-    for (int i = 0; i < 8; ++i) rows = rows && (!(i < 4 ? p->q_heads : p->k_heads) || strides[i] * size % 16 == 0);
+    for (int i = 0; i < 8; ++i) {
+        const int64_t heads = i < 4 ? p->q_heads : p->k_heads;           // (a dimension of one entry has any stride)
+        rows = rows && (!heads || (i % 2 ? heads : p->tokens) == 1 || strides[i] * size % 16 == 0);
+    }
     for (const void *q : {p->q, static_cast<const void *>(p->q_out)}) rows = rows && (!p->q_heads || aligned(q, 16));
     for (const void *k : {p->k, static_cast<const void *>(p->k_out)}) rows = rows && (!p->k_heads || aligned(k, 16));
     a.in[0] = p->q, a.in[1] = p->k, a.out[0] = p->q_out, a.out[1] = p->k_out;

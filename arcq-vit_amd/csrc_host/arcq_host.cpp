@@ -1202,7 +1202,7 @@ inline bool differentiable(const Tensor &t) { return (c10::GradMode::is_enabled(
 // [rows, heads, dim] of 16 bits whose rows lie whole on 16-byte boundaries.
 inline bool rows16(const Tensor &t)
 {
-    return t.dim() == 3 && t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned16(t);
+    return t.dim() == 3 && t.stride(2) == 1 && (t.size(0) <= 1 || t.stride(0) % 8 == 0) && (t.size(1) <= 1 || t.stride(1) % 8 == 0) && aligned16(t);
 }
 inline void *raw(const Tensor &t) { return const_cast<void *>(t.const_data_ptr()); }
 

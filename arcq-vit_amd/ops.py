@@ -881,7 +881,8 @@ def _pages_args(pages) -> "tuple[_lib.KvPages, list]":
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """``[rows, heads, dim]`` of 16 bits whose rows lie whole on 16-byte boundaries: ``t`` itself or a copy."""
-    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0:
+    # (a dimension of one entry has any stride)
+    if t.stride(2) == 1 and all(t.shape[i] <= 1 or t.stride(i) % 8 == 0 for i in (0, 1)) and t.data_ptr() % 16 == 0:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
