@@ -13,7 +13,8 @@
 // Softmax.  One pass: the maximum m and the sum are per lane and row, in 32 bits, and the outputs are rescaled when m grows.
 //
 // Bounds.  Few rows (a step): the pages are read once at the rate at which memory is read: 6.0 TB/s, of which the 64 sequences
-// above reach 5.4 (1 010 MB, 187 us), the FP8 pages of two of 130 000 keys 5.2.  Many rows: the matrix pipe.  A 32 x 32 x 16 instruction
+// above reach 5.4 (1 010 MB, 187 us, the join's launch of 5 us included), the FP8 pages of two of 130 000 keys 5.3 (537 MB, 101 us; 5.6 in
+// the first launch alone).  Many rows: the matrix pipe.  A 32 x 32 x 16 instruction
 // takes 32 clocks of its SIMD, the softmax between two products about as long in vector instructions, and what a wave leaves idle the other
 // one of its SIMD fills only in part: a chunk of 2 048 tokens behind 6 000 keys (32 heads of 128, 8 key heads) 238 us, 990 TFLOP/s, the
 // matrix pipe busy 46 % of all clocks; a library product of 8 192^3 reaches 1 210.
@@ -48,7 +49,8 @@ constexpr float kNegInf = -__builtin_inff();
 // A row's maximum: kNegInf if it sees no key (its result is zero), kLowest if it sees some and none has a score above minus infinity (0 / 0).
 constexpr float kLowest = -3.402823466e38f;
 __device__ __forceinline__ float row_maximum(float m, bool sees) { return sees ? fmaxf(m, kLowest) : m; }
-// How far a score may be above the reference (in powers of two) before that follows, in the kernel of many rows.
+// How far a score may be above the reference (in powers of two) before that follows, in the kernel of many rows.  (0: a chunk of 2 048 tokens 4 %
+// slower; 16, which only bf16 probabilities have room for: no faster.)
 constexpr int kSlack = 6;
 
 // Division of 0 .. 2^30 - 1 by a number known on the host: l = ceil(log2 d), m = ceil(2^(30 + l) / d) < 2^32; m d exceeds 2^(30 + l) by less
@@ -70,7 +72,8 @@ struct Divide {
 // The factors of probabilities (2^shift) and of FP8 values whose exponents go to the probabilities (value_scale); back: the latter's inverse, for
 // the result.  bf16, sums of up to 2^n keys, probabilities of up to 2^(shift + slack):
 //   16-bit pages  2^n * 2^(shift + slack) * |v| < 2^128 / 2
-//   FP8           P = p 2^e is a bf16 number at both ends of e, 2^(119 + 8) and 2^(-110 + 8 - slack) less 18 powers;  2^n * 2^127 * 448 * value_scale < 2^128
+//   FP8           P = p 2^e is a bf16 number at both ends of e, 2^(119 + 8) and 2^(-110 + 8 - slack) less 18 powers;
+//                 2^n * 2^127 * 448 * value_scale < 2^128
 struct Range {
     float shift, value_scale, back;
     Range(int dtype, bool f8, int64_t keys, int slack)
@@ -391,7 +394,8 @@ __device__ __forceinline__ void store_rows(const PagedArgs &a, const Item &t, in
 }
 
 // A tile by the definition, row by row and key by key: for one that has values which are not finite where some of its rows must not see
-// them, or a page that does not exist.  A wave takes a row at a time, 64 keys' scores at once, a lane the dims lane + 64 i.
+// them, or a page that does not exist.  A wave takes a row at a time, 64 keys' scores at once, a lane the dims lane + 64 i.  It is for tiles
+// that hardly ever are, and slow: a chunk of 2 048 tokens behind 6 000 keys, 32 heads of 128, a NaN in its last value: 58 ms, without it 0.24.
 template <typename T, bool F8, int D, int TILE, int SHIFT, int WAVES>
 __device__ __forceinline__ void careful_tile(const PagedArgs &a, const Item &t, int kv, int wave, int lane)
 {
@@ -733,7 +737,8 @@ paged_rows_kernel(const PagedArgs a)
 // 128 rows read a block from L2 once for four waves, 64 KB of LDS (128 dims) leave two workgroups a compute unit, and 256 registers a wave
 // hold the queries, 64 keys' scores and the outputs: hence exactly two waves a SIMD (`amdgpu_waves_per_eu`; told "two at least" the
 // compiler spilled to reach three).  Beside the products and the softmax a block's addresses count (at 64 dims as many instructions as
-// either): a lane holds the place of one of the next 64 blocks, or of one of 16 tokens of the next 16, and a wave's loads share an address.  256 rows and eight waves: 269 us against 249 for the chunk of 2 048 tokens; the next block's scores
+// either): a lane holds the place of one of the next 64 blocks, or of one of 16 tokens of the next 16, and a wave's loads share an
+// address.  256 rows and eight waves: 269 us against 249 for the chunk of 2 048 tokens; the next block's scores
 // begun before this one's softmax 266 against 259; row sums by dot products 256 against 249; three waves with one buffer each for
 // keys and values: spills; the next block's loads behind the scores' products, or `s_setprio` around those: within 1 %.
 constexpr int kTileRows = 128;
@@ -977,7 +982,8 @@ paged_tile_kernel(const PagedArgs a)
         if (careful) break;                       // (the same in all waves)
         if (base >= wave_hi || base + 64 <= wave_lo) continue;
         if constexpr (kScaleValues<T, F8>) {
-            // A lane a pair of tokens, for all lanes of the wave: each for its own 32 tokens took 42 us in place of 39 (64 dims, a window of 1 000).
+            // A lane a pair of tokens, for all lanes of the wave: each lane for its own 32 took 41.8 us in place of 37.5 (ragged chunks, 64 dims,
+            // a window of 1 000 keys), conversions of one value at a time with its own scale 49.6.
             // (What lies outside of the tile's keys, where an exponent may be anything: zero times zero.)
             const int first = base + 2 * lr;
             half2_t two = scales_of(*reinterpret_cast<const uint16_t *>(block + 2 * HALF + 64 + 2 * lr), false);

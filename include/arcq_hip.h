@@ -467,7 +467,8 @@ int arcq_qk_norm_rotary(const arcq_qk_norm_rotary_args *a, void *stream);
  * contiguous runs of them:
  *   k [num_pages, heads, head_dim / w, page_size, w]      v [num_pages, heads, page_size / w, head_dim, w]
  * ARCQ_FP8: a value is 2^exponent times the E4M3 value, k_exponents / v_exponents int8 [num_pages, heads, page_size]: one
- * for each token and head; they are read as the 16-bit type that they were written from.  Slot p * page_size + j is place j of page p.  head_dim: a multiple of 16, at most 256.
+ * for each token and head; they are read as the 16-bit type that they were written from.  Slot p * page_size + j is place j
+ * of page p.  head_dim: a multiple of 16, at most 256.
  * All four 16-byte aligned. */
 typedef struct arcq_kv_pages {
     void *k, *v;
@@ -502,7 +503,8 @@ int arcq_kv_cache_read(const arcq_kv_cache_args *a, void *stream);
  *   q, out [tokens, q_heads, head_dim] of dtype ARCQ_F16 / ARCQ_BF16 (16-bit pages: theirs), strides in elements, rows
  *   16-byte aligned; page_table int32 [sequences, table_width], table_stride elements between rows; q_offsets int32
  *   [sequences + 1], ascending from 0; kv_lengths int32 [sequences].  head_dim 32, 64, 96, 128 or 256.
- * fp32 scores, softmax and accumulation, the probabilities rounded to dtype before the second product; keys are read within
+ * fp32 scores, softmax and accumulation, the probabilities rounded to dtype before the second product; sums over values stay
+ * finite wherever the values are.  A token whose keys all have a score of minus infinity gets NaN.  Keys are read within
  * the table and the pages only: an entry outside of [0, num_pages) is not followed and gives the tokens that see it NaN.
  * workspace: arcq_attention_paged_workspace(a) bytes of scratch, 16-byte aligned (0: none).  scale > 0. */
 typedef struct arcq_attention_paged_args {
