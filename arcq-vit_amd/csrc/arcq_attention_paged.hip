@@ -40,6 +40,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace arcq {
 namespace {
@@ -52,6 +53,7 @@ __device__ __forceinline__ float row_maximum(float m, bool sees) { return sees ?
 // How far a score may be above the reference (in powers of two) before that follows, in the kernel of many rows.  (0: a chunk of 2 048 tokens 4 %
 // slower; 16, which only bf16 probabilities have room for: no faster.)
 constexpr int kSlack = 6;
+constexpr int kShiftF16 = 8;
 
 // Division of 0 .. 2^30 - 1 by a number known on the host: l = ceil(log2 d), m = ceil(2^(30 + l) / d) < 2^32; m d exceeds 2^(30 + l) by less
 // than 2^l, n times that by less than 2^(30 + l), so the quotient is exact.
@@ -80,7 +82,7 @@ struct Range {
     {
         const int n = log2_of(std::max<int64_t>(keys, 1));
         const bool scaled = dtype == ARCQ_BF16 && f8;
-        shift = static_cast<float>(dtype == ARCQ_F16 ? 8 : f8 ? 8 - slack : -(n + slack + 1));
+        shift = static_cast<float>(dtype == ARCQ_F16 ? kShiftF16 : f8 ? 8 - slack : -(n + slack + 1));
         value_scale = scaled ? std::ldexp(1.0f, -(n + 9)) : 1.0f;
         back = scaled ? std::ldexp(1.0f, n + 9) : 1.0f;
     }
@@ -103,6 +105,11 @@ struct PagedArgs {
     float shift, value_scale, back;  // Range
     Divide by_group, by_kv_heads, by_q_heads;
 };
+
+// (fp16's are constants: as arguments a step of four short sequences took 7.44 us in place of 7.35)
+template <typename T> constexpr bool kConstantRange = std::is_same<T, _Float16>::value;
+template <typename T> __device__ __forceinline__ float shift_of(const PagedArgs &a) { return kConstantRange<T> ? static_cast<float>(kShiftF16) : a.shift; }
+template <typename T> __device__ __forceinline__ float back_of(const PagedArgs &a) { return kConstantRange<T> ? 1.0f : a.back; }
 
 __device__ __forceinline__ int offset_of(const PagedArgs &a, int b) { return min(max(a.q_offsets[b], 0), static_cast<int>(a.tokens)); }
 
@@ -369,7 +376,7 @@ __device__ __forceinline__ void store_rows(const PagedArgs &a, const Item &t, in
     const int tok = a.by_group(row), head = kv * a.group + row - tok * a.group;
     const int64_t token = static_cast<int64_t>(t.token0) + tok;
     if (t.parts == 1) {
-        const float inv = m == kNegInf ? 0.0f : a.back / l;
+        const float inv = m == kNegInf ? 0.0f : back_of<T>(a) / l;
         unsigned char *dst = a.out + token * a.out_token + head * a.out_head;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
@@ -436,7 +443,7 @@ __device__ __forceinline__ void careful_tile(const PagedArgs &a, const Item &t, 
             for (int x = 32; x; x >>= 1) bm = fmaxf(bm, __shfl_xor(bm, x));
             const float m_new = fmaxf(m, bm), base2 = m_new == kNegInf ? 0.0f : m_new;
             const float alpha = __builtin_amdgcn_exp2f(m - base2);
-            const float p = lane < n ? __builtin_amdgcn_exp2f(s - base2 + a.shift) : 0.0f;
+            const float p = lane < n ? __builtin_amdgcn_exp2f(s - base2 + shift_of<T>(a)) : 0.0f;
             float sum = p;
 #pragma unroll
             for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
@@ -456,7 +463,7 @@ __device__ __forceinline__ void careful_tile(const PagedArgs &a, const Item &t, 
         }
         m = row_maximum(m, sees);
         const bool alone = t.parts == 1;
-        const float inv = m == kNegInf ? 0.0f : a.back / l;
+        const float inv = m == kNegInf ? 0.0f : back_of<T>(a) / l;
         T *dst = reinterpret_cast<T *>(a.out + token * a.out_token + head * a.out_head);
         const int64_t at = part_row<TILE>(a, t, kv, t.part, r) * D;
 #pragma unroll
@@ -640,7 +647,7 @@ paged_rows_kernel(const PagedArgs a)
                 for (int v = 0; v < 16; ++v) o[i][v] *= alpha;
             m = m_new;
         }
-        const float shift = a.shift - base2;
+        const float shift = shift_of<T>(a) - base2;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.c2, shift));
@@ -709,7 +716,7 @@ paged_rows_kernel(const PagedArgs a)
         const int rtok = a.by_group(rr), rhead = kv * a.group + rr - rtok * a.group;
         const int64_t token = static_cast<int64_t>(t.token0) + rtok;
         const bool alone = t.parts == 1;
-        const float inv = alone ? (mm == kNegInf ? 0.0f : a.back / total) : 1.0f;
+        const float inv = alone ? (mm == kNegInf ? 0.0f : back_of<T>(a) / total) : 1.0f;
         const int64_t at = part_row<32>(a, t, kv, t.part, r);
         float *po = alone ? nullptr : a.part_o + at * D;
         unsigned char *dst = a.out + token * a.out_token + rhead * a.out_head;
@@ -1033,7 +1040,7 @@ paged_tile_kernel(const PagedArgs a)
                 for (int v = 0; v < 16; ++v) o[i][v] *= alpha;
             m = m_new;
         }
-        const float shift = a.shift - (m == kNegInf ? 0.0f : m);       // (a row that has seen nothing yet)
+        const float shift = shift_of<T>(a) - (m == kNegInf ? 0.0f : m);       // (a row that has seen nothing yet)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             u32x4_t pf[2];
@@ -1124,7 +1131,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] += o[i];
     }
-    const float inv = mm == kNegInf ? 0.0f : a.back / total;
+    const float inv = mm == kNegInf ? 0.0f : back_of<T>(a) / total;
     const int head = static_cast<int>(at - token * a.q_heads);
     u32x2_t w;
     w[0] = pack2(sum[0] * inv, sum[1] * inv, T{});
