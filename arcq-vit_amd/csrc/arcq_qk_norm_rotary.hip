@@ -303,13 +303,21 @@ __global__ void __launch_bounds__(256) rotary_rows_kernel(const RotaryArgs a)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) c[i] = 1.0f, s[i] = 0.0f;
             }
-            // (what does not turn is taken as it is: turned by an angle of zero an infinity would make its partner NaN, and -0 become 0)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int p = HOW == kNeighbours ? 2 * i : i, q = HOW == kNeighbours ? 2 * i + 1 : 8 + i;
-                const bool pair = HOW == kNeighbours ? 8 * lane + i < a.pairs : turns;
-                y[p] = pair ? __builtin_fmaf(-v[q], s[i], v[p] * c[i]) : v[p];
-                y[q] = pair ? __builtin_fmaf(v[p], s[i], v[q] * c[i]) : v[q];
+                y[p] = __builtin_fmaf(-v[q], s[i], v[p] * c[i]);
+                y[q] = __builtin_fmaf(v[p], s[i], v[q] * c[i]);
+            }
+            // What does not turn is taken as it is: turned by an angle of zero an infinity would make its partner NaN, and -0 become 0.
+            if (2 * a.pairs < a.dim) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int p = HOW == kNeighbours ? 2 * i : i, q = HOW == kNeighbours ? 2 * i + 1 : 8 + i;
+                    const bool pair = HOW == kNeighbours ? 8 * lane + i < a.pairs : turns;
+                    y[p] = pair ? y[p] : v[p];
+                    y[q] = pair ? y[q] : v[q];
+                }
             }
         }
         if (busy)
