@@ -106,10 +106,23 @@ struct PagedArgs {
     Divide by_group, by_kv_heads, by_q_heads;
 };
 
-// (fp16's are constants: as arguments a step of four short sequences took 7.44 us in place of 7.35)
-template <typename T> constexpr bool kConstantRange = std::is_same<T, _Float16>::value;
-template <typename T> __device__ __forceinline__ float shift_of(const PagedArgs &a) { return kConstantRange<T> ? static_cast<float>(kShiftF16) : a.shift; }
-template <typename T> __device__ __forceinline__ float back_of(const PagedArgs &a) { return kConstantRange<T> ? 1.0f : a.back; }
+// A kernel's factors: constants for fp16, else read with its first arguments (where they are used first they cost short steps a round trip each:
+// a step of four short sequences 7.44 us in place of 7.35).
+template <typename T, bool F8>
+struct Factors {
+    float shift = kShiftF16, value_scale = 1.0f, back = 1.0f;
+    __device__ __forceinline__ explicit Factors(const PagedArgs &a)
+    {
+        if constexpr (!std::is_same<T, _Float16>::value) {
+            shift = a.shift;
+            asm volatile("" : "+s"(shift));
+            if constexpr (F8) {
+                value_scale = a.value_scale, back = a.back;
+                asm volatile("" : "+s"(value_scale), "+s"(back));
+            }
+        }
+    }
+};
 
 __device__ __forceinline__ int offset_of(const PagedArgs &a, int b) { return min(max(a.q_offsets[b], 0), static_cast<int>(a.tokens)); }
 
@@ -371,12 +384,12 @@ __device__ __forceinline__ void say_parts(const PagedArgs &a, const Item &t, int
 }
 // A lane's half of its row: the result, or the part's sums.
 template <typename T, int D, int TILE = 32>
-__device__ __forceinline__ void store_rows(const PagedArgs &a, const Item &t, int kv, int row, int lh, float m, float l, const float16_t (&o)[D / 32])
+__device__ __forceinline__ void store_rows(const PagedArgs &a, float back, const Item &t, int kv, int row, int lh, float m, float l, const float16_t (&o)[D / 32])
 {
     const int tok = a.by_group(row), head = kv * a.group + row - tok * a.group;
     const int64_t token = static_cast<int64_t>(t.token0) + tok;
     if (t.parts == 1) {
-        const float inv = m == kNegInf ? 0.0f : back_of<T>(a) / l;
+        const float inv = m == kNegInf ? 0.0f : back / l;
         unsigned char *dst = a.out + token * a.out_token + head * a.out_head;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
@@ -404,7 +417,7 @@ __device__ __forceinline__ void store_rows(const PagedArgs &a, const Item &t, in
 // them, or a page that does not exist.  A wave takes a row at a time, 64 keys' scores at once, a lane the dims lane + 64 i.  It is for tiles
 // that hardly ever are, and slow: a chunk of 2 048 tokens behind 6 000 keys, 32 heads of 128, a NaN in its last value: 58 ms, without it 0.24.
 template <typename T, bool F8, int D, int TILE, int SHIFT, int WAVES>
-__device__ __forceinline__ void careful_tile(const PagedArgs &a, const Item &t, int kv, int wave, int lane)
+__device__ __forceinline__ void careful_tile(const PagedArgs &a, const Factors<T, F8> &f, const Item &t, int kv, int wave, int lane)
 {
     constexpr int W = F8 ? 16 : 8, SZ = F8 ? 1 : 2, PER = (D + 63) / 64;
     const int32_t *table = a.table + t.b * a.table_stride;
@@ -443,7 +456,7 @@ __device__ __forceinline__ void careful_tile(const PagedArgs &a, const Item &t, 
             for (int x = 32; x; x >>= 1) bm = fmaxf(bm, __shfl_xor(bm, x));
             const float m_new = fmaxf(m, bm), base2 = m_new == kNegInf ? 0.0f : m_new;
             const float alpha = __builtin_amdgcn_exp2f(m - base2);
-            const float p = lane < n ? __builtin_amdgcn_exp2f(s - base2 + shift_of<T>(a)) : 0.0f;
+            const float p = lane < n ? __builtin_amdgcn_exp2f(s - base2 + f.shift) : 0.0f;
             float sum = p;
 #pragma unroll
             for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
@@ -458,12 +471,12 @@ __device__ __forceinline__ void careful_tile(const PagedArgs &a, const Item &t, 
                 const unsigned char *v = a.vp + (sj - oj) * (D * SZ) + oj / W * D * 16 + oj % W * SZ;
 #pragma unroll
                 for (int i = 0; i < PER; ++i)
-                    if (lane + 64 * i < D) o[i] = __builtin_fmaf(pj, value(v + (lane + 64 * i) * 16, ej) * a.value_scale, o[i]);
+                    if (lane + 64 * i < D) o[i] = __builtin_fmaf(pj, value(v + (lane + 64 * i) * 16, ej) * f.value_scale, o[i]);
             }
         }
         m = row_maximum(m, sees);
         const bool alone = t.parts == 1;
-        const float inv = m == kNegInf ? 0.0f : back_of<T>(a) / l;
+        const float inv = m == kNegInf ? 0.0f : f.back / l;
         T *dst = reinterpret_cast<T *>(a.out + token * a.out_token + head * a.out_head);
         const int64_t at = part_row<TILE>(a, t, kv, t.part, r) * D;
 #pragma unroll
@@ -495,6 +508,7 @@ paged_rows_kernel(const PagedArgs a)
     const int tid = threadIdx.x, lane = tid & 63, wave = WAVES == 1 ? 0 : tid >> 6;
     const int lr = lane & 31, lh = lane >> 5;
     const int place = a.by_kv_heads(blockIdx.x), kv = blockIdx.x - place * a.kv_heads;
+    const Factors<T, F8> range(a);
     Item t;
     if (!find_item<32, 5>(a, place, lane, t)) return;
     const int k0 = t.k0, k1 = t.k1;
@@ -509,6 +523,7 @@ paged_rows_kernel(const PagedArgs a)
         hi = min(max(t.len - t.queries + tok + 1, 0), t.len);
         if (a.window) lo = max(t.len - t.queries + tok + 1 - a.window, 0);
     }
+    const uint64_t sees = __ballot(hi > lo);        // (a bit a lane: 36 sequences of 7 736 keys, 2 heads of 256, 152 us; by the bounds, kept in registers to the end, 155)
     u32x4_t qf[KF];
     {
         const unsigned char *src = a.q + static_cast<int64_t>(t.token0 + tok) * a.q_token + head * a.q_head;
@@ -621,7 +636,7 @@ paged_rows_kernel(const PagedArgs a)
             if constexpr (F8) {
 #pragma unroll
                 for (int i = 0; i < NB; ++i) keep_tokens<F8>(vreg[i], base + 16 * lh, t.lo, t.hi);
-                keep_tokens<F8>(vexp, base + 16 * lh, t.lo, t.hi);
+                if constexpr (kScaleValues<T, F8>) keep_tokens<F8>(vexp, base + 16 * lh, t.lo, t.hi);
             } else {
 #pragma unroll
                 for (int i = 0; i < 2 * NB; ++i) keep_tokens<F8>(vreg[i], base + 16 * (i / NB) + 8 * lh, t.lo, t.hi);
@@ -647,7 +662,7 @@ paged_rows_kernel(const PagedArgs a)
                 for (int v = 0; v < 16; ++v) o[i][v] *= alpha;
             m = m_new;
         }
-        const float shift = shift_of<T>(a) - base2;
+        const float shift = range.shift - base2;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.c2, shift));
@@ -665,7 +680,7 @@ paged_rows_kernel(const PagedArgs a)
             for (int e = 0; e < 4; ++e) pf[i][e] = pack2(s[8 * i + 2 * e], s[8 * i + 2 * e + 1], T{});
         auto value = [&](int i, int j) {
             if constexpr (kScaleValues<T, F8>) return widen_each(vreg[j][2 * i], vreg[j][2 * i + 1], vscale + 4 * i);
-            else if constexpr (F8) return widen(vreg[j][2 * i], vreg[j][2 * i + 1], a.value_scale, T{});
+            else if constexpr (F8) return widen(vreg[j][2 * i], vreg[j][2 * i + 1], range.value_scale, T{});
             else return vreg[i * NB + j];
         };
 #pragma unroll
@@ -676,13 +691,13 @@ paged_rows_kernel(const PagedArgs a)
     }
     l += __shfl_xor(l, 32);
     if (WAVES == 1 ? careful : __syncthreads_or(careful) != 0) {
-        careful_tile<T, F8, D, 32, 5, WAVES>(a, t, kv, wave, lane);
+        careful_tile<T, F8, D, 32, 5, WAVES>(a, range, t, kv, wave, lane);
         return;
     }
 
-    m = row_maximum(m, hi > lo);
+    m = row_maximum(m, (sees >> lane) & 1);
     if constexpr (WAVES == 1) {
-        if (live) store_rows<T, D>(a, t, kv, row, lh, m, l, o);
+        if (live) store_rows<T, D>(a, range.back, t, kv, row, lh, m, l, o);
         return;
     } else {
         // ---- the waves' maxima, sums and outputs ----
@@ -716,7 +731,7 @@ paged_rows_kernel(const PagedArgs a)
         const int rtok = a.by_group(rr), rhead = kv * a.group + rr - rtok * a.group;
         const int64_t token = static_cast<int64_t>(t.token0) + rtok;
         const bool alone = t.parts == 1;
-        const float inv = alone ? (mm == kNegInf ? 0.0f : back_of<T>(a) / total) : 1.0f;
+        const float inv = alone ? (mm == kNegInf ? 0.0f : range.back / total) : 1.0f;
         const int64_t at = part_row<32>(a, t, kv, t.part, r);
         float *po = alone ? nullptr : a.part_o + at * D;
         unsigned char *dst = a.out + token * a.out_token + rhead * a.out_head;
@@ -820,6 +835,7 @@ paged_tile_kernel(const PagedArgs a)
     const int lr = lane & 31, lh = lane >> 5;
     half2_t *wave_scales = scales[kScaleValues<T, F8> ? wave : 0];
     const int place = a.by_kv_heads(blockIdx.x), kv = blockIdx.x - place * a.kv_heads;
+    const Factors<T, F8> range(a);
     Item t;
     if (!find_item<kTileRows, 6>(a, place, lane, t)) return;
     const int k0 = t.k0, k1 = t.k1;
@@ -1040,7 +1056,7 @@ paged_tile_kernel(const PagedArgs a)
                 for (int v = 0; v < 16; ++v) o[i][v] *= alpha;
             m = m_new;
         }
-        const float shift = shift_of<T>(a) - (m == kNegInf ? 0.0f : m);       // (a row that has seen nothing yet)
+        const float shift = range.shift - (m == kNegInf ? 0.0f : m);       // (a row that has seen nothing yet)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             u32x4_t pf[2];
@@ -1066,7 +1082,7 @@ paged_tile_kernel(const PagedArgs a)
                     for (int i = 0; i < 2; ++i) {
                         u32x4_t v;
                         if constexpr (kScaleValues<T, F8>) v = widen_each(w[2 * i], w[2 * i + 1], vscale + 4 * i);
-                        else v = widen(w[2 * i], w[2 * i + 1], a.value_scale, T{});
+                        else v = widen(w[2 * i], w[2 * i + 1], range.value_scale, T{});
                         o[j] = mfma(v, pf[i], o[j], T{});
                     }
                 } else {
@@ -1079,11 +1095,11 @@ paged_tile_kernel(const PagedArgs a)
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (careful) {
-        careful_tile<T, F8, D, kTileRows, 6, 4>(a, t, kv, wave, lane);
+        careful_tile<T, F8, D, kTileRows, 6, 4>(a, range, t, kv, wave, lane);
         return;
     }
     l += __shfl_xor(l, 32);
-    if (live) store_rows<T, D, kTileRows>(a, t, kv, row, lh, row_maximum(m, hi > lo), l, o);
+    if (live) store_rows<T, D, kTileRows>(a, range.back, t, kv, row, lh, row_maximum(m, hi > lo), l, o);
 }
 
 // ---- the parts of a row, joined: a workgroup has a row, groups of D / 4 threads take the parts in turn and are added in their order (the
@@ -1131,7 +1147,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] += o[i];
     }
-    const float inv = mm == kNegInf ? 0.0f : back_of<T>(a) / total;
+    const float inv = mm == kNegInf ? 0.0f : a.back / total;
     const int head = static_cast<int>(at - token * a.q_heads);
     u32x2_t w;
     w[0] = pack2(sum[0] * inv, sum[1] * inv, T{});
