@@ -817,8 +817,8 @@ struct Block {
     static constexpr int SIZE = 2 * HALF + (F8 ? 256 : 0);
 };
 // Waves a SIMD that the compiler makes registers last for.  Up to 64 dims four, where that spills nothing (64 sequences of up to 512 new tokens
-// and 4 096 keys, 16 heads: 64 dims 237 -> 221 us, 32 dims 186 -> 166, FP8 257 -> 222; FP8 pages of 64 dims would spill, 42 -> 46 us with a
-// window of 1 000).
+// and 4 096 keys, 16 heads: 64 dims 237 -> 221 us, 32 dims 186 -> 166, FP8 257 -> 222; FP8 pages of 64 dims would spill, 37.7 -> 38.6 us with
+// a window of 1 000).
 template <bool F8, int D> constexpr int kTileWaves = D <= 32 || (D <= 64 && !F8) ? 4 : D <= 128 ? 2 : 1;
 
 template <typename T, bool F8, int D, bool ONE_PAGE>

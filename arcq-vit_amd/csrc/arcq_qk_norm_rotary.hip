@@ -8,7 +8,7 @@
 // at position 2^20, where a 32-bit product is off by a tenth of a radian; the nearest quarter goes the same way, and sine and cosine
 // of what is left (an eighth of a turn at most) are short polynomials in 32 bits.
 //
-// Bound by memory: 16 384 tokens of 40 heads of 128 (336 MB) 66.4 us, 5.1 TB/s, a copy's rate; a step of 64 tokens 5.6 us, a launch and
+// Bound by memory: 16 384 tokens of 40 heads of 128 (336 MB) 66.0 us, 5.1 TB/s, a copy's rate; a step of 64 tokens 5.6 us, a launch and
 // one round trip.  The angles are not: in 64 bits they cost as much as the rest where every head computes its own (170 us), so a
 // workgroup computes each token's once for all its heads.
 #include "arcq_gemm.h"
